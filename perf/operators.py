@@ -11,9 +11,7 @@ Five kinds of case, all over pages of 64 tokens named by a block table:
 The latent row is 416 bytes: 512 e2m1 codes (value 2j in the low nibble of byte j), 32 e4m3 scales (one per
 16 values, amax / 6), 64 bf16 roped key dims.
 """
-import pathlib
 import random
-import sys
 
 import numpy as np
 import torch
@@ -26,7 +24,6 @@ IDX_PAGE = PAGE * 132
 WORKSPACE = 40 << 20   # the attention's workspace: two partial row tiles an SM
 SCALE = 256 ** -0.5    # the score scale of 192 + 64 dims a head
 DEV = "cuda"
-PACKAGE = str(pathlib.Path(__file__).resolve().parents[1] / "kern-glm53_b200")
 
 
 # ------------------------------------------------------------------------------------------ cases
@@ -364,8 +361,6 @@ def run(s):
     if not own:
         return {"append": _plain_append, "attn": _plain_attn, "picks": _plain_picks, "weights": _plain_weights,
                 "evict": _plain_evict}[kind](s)
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
     import glmkv
     T = s["T"]
     if kind == "append":
