@@ -665,7 +665,9 @@ __device__ __forceinline__ void a4_run(const A4Args& a) {
     const bool any = g.kt0 < ke;
     references(g.rt0);
     a4_sync();
-    if (tid == 0) step_walk(segs[at ^ 1]);  // the segment after this: known to all from the next barrier on
+    // The segment after this, for all to read past the next barrier: in a first tile's raise, in begin(), or, for the
+    // weights of a tile prepared before, the one after the wait for its scores, which the walk is stepped under.
+    if (tid == 0) step_walk(segs[at ^ 1]);
     [[maybe_unused]] float sum[32];
     if constexpr (MODE != A4_WEIGHTS) {
 #pragma unroll
@@ -700,6 +702,8 @@ __device__ __forceinline__ void a4_run(const A4Args& a) {
               references(rt);
               a4_sync();
             }
+          } else if (kt == g.kt0) {
+            a4_sync();  // the segment after this is read below, and a tile of one row tile has no barrier before that
           }
         }
         masked = slot < 0 || k >= lim[0];

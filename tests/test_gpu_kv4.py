@@ -239,6 +239,42 @@ def test_weights(cuda, lens, qlens, heads):
     assert abs(want.sum() - rows) < 1e-3 * max(rows, 1)
 
 
+def _short_sequences(kind):
+    """Batches where every CTA walks several sequences, each of a few tiles or of one."""
+    if kind == "one tile":
+        return [70] * 1000, [1] * 1000
+    rng = np.random.default_rng(600)
+    lens = rng.choice([0, 1, 64, 128, 129, 256, 300, 384, 640], 600).tolist()
+    return lens, rng.choice([0, 1, 1, 1, 2], 600).tolist()
+
+
+@pytest.mark.parametrize("kind", ["one tile", "mixed"])
+@pytest.mark.parametrize("heads", [8, 64])
+def test_many_short_sequences_a_cta(cuda, kind, heads):
+    """A sequence's first tile is prepared before it begins, from what the walk says of it: no warp may read that
+    before the walk is there. Attention and weights, several times over."""
+    import glmkv
+    from kv4_case import Kv4Case
+
+    c = Kv4Case(*_short_sequences(kind), heads, seed=heads)
+    d = c.device(torch, cuda)
+    c.attn(d)
+    out, lse = d["out"].clone(), d["lse"].clone()
+    accs = []
+    for _ in range(6):
+        c.attn(d)
+        assert torch.equal(out, d["out"]) and torch.equal(lse, d["lse"])
+        accs.append(torch.zeros(c.n_pages * 64, device=cuda))
+        c.weights(d, accs[-1])
+    torch.cuda.synchronize()
+    assert glmkv.fault_flags() == 0
+    c.check_attn(_np(out), _np(lse))
+    want, tol = c.want_weights(_np(lse).astype(np.float64))
+    err = np.abs(_np(accs[0]).astype(np.float64) - want)
+    assert np.all(err <= tol + want * 2.0 ** -24), np.max(err)
+    assert all(torch.equal(accs[0], a) for a in accs[1:])
+
+
 # ------------------------------------------------------------------------------------------ as a program uses them
 
 def test_bad_pages_and_picks_are_skipped_and_flagged(cuda):
