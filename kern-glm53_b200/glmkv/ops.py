@@ -110,12 +110,20 @@ def plan(cu, seq_lens, nseq, pos, ks, ke, klen, row_seq, zero, T, stream=None):
               _ptr(row_seq, "i32", "row_seq"), _ptr(zero, "i32", "zero"), int(T), _stream(stream))
 
 
-_PREP = {"fp8": "_fp8", "fp4": "_fp4"}  # anything else appends bf16 rows
+_PREP = {"fp8": "glmkv_mla_prep_fp8", "bf16": "glmkv_mla_prep", "fp4": "glmkv_mla_prep_fp4"}
+
+
+def _row_bytes(kv_dtype):
+    """Bytes of a latent row. A name that is no format is refused: the widest row, in a cache of the
+    narrowest, is written far past its end."""
+    if kv_dtype not in traffic.KV_ROW:
+        raise ValueError(f"kv_dtype {kv_dtype!r}: one of {sorted(traffic.KV_ROW)}")
+    return traffic.KV_ROW[kv_dtype]
 
 
 def _prep(kv_dtype, x, lda, g_q, g_kv, rope, pos, slot, kv, idx, ik_w, ik_b, qq, qsf, sf_rows, T, stream):
-    name = "glmkv_mla_prep" + _PREP.get(kv_dtype, "")
-    _lib.call(name, _ptr(x, "bf16", "x"), int(lda), _ptr(g_q, "bf16", "g_q"), _ptr(g_kv, "bf16", "g_kv"),
+    _row_bytes(kv_dtype)
+    _lib.call(_PREP[kv_dtype], _ptr(x, "bf16", "x"), int(lda), _ptr(g_q, "bf16", "g_q"), _ptr(g_kv, "bf16", "g_kv"),
               _ptr(rope, "bf16", "rope"), _ptr(pos, "i32", "pos"), _ptr(slot, "i64", "slot"), _ptr(kv, "u8", "kv"),
               _ptr(idx, "u8", "idx"), _ptr(ik_w, "bf16", "ik_w"), _ptr(ik_b, "bf16", "ik_b"), _ptr(qq, "u8", "qq"),
               _ptr(qsf, "u8", "qsf"), int(sf_rows), int(T), _stream(stream))
@@ -193,11 +201,10 @@ def evict_plan(acc, pos, n_pages, block_table, max_pages, seq_lens, seen, nseq, 
 def evict_rows(moves, n_moves, nseq, budget, n_pages, kv, idx, acc, pos, *, kv_dtype="fp4", stream=None):
     """The plan's moves in a latent cache of `kv_dtype` rows, an indexer cache, the running weights and the
     positions (None: left as it is)."""
-    if kv_dtype not in traffic.KV_ROW:
-        raise ValueError(f"kv_dtype {kv_dtype!r}: one of {sorted(traffic.KV_ROW)}")
+    row = _row_bytes(kv_dtype)
     _here(moves, n_moves, kv, idx, acc, pos)
     _lib.call("glmkv_evict_rows", _ptr(moves, "i32", "moves"), _ptr(n_moves, "i32", "n_moves"), int(nseq), int(budget),
-              int(n_pages), _ptr(kv, "u8", "kv"), traffic.KV_ROW[kv_dtype], _ptr(idx, "u8", "idx"), _ptr(acc, "f32", "acc"),
+              int(n_pages), _ptr(kv, "u8", "kv"), row, _ptr(idx, "u8", "idx"), _ptr(acc, "f32", "acc"),
               _ptr(pos, "i32", "pos"), _stream(stream))
 
 

@@ -224,6 +224,8 @@ def random_latent_pages(rng, n_pages, kv_dtype="fp8"):
     spanning 2^-20 .. 2^4, bf16 k_pe ~ N(0, 1). bf16 pools hold N(0, 1) values."""
     if kv_dtype == "bf16":
         return bf16_bits(rng.standard_normal(n_pages * PAGE * 576, dtype=np.float32)).view(np.uint8)
+    if kv_dtype != "fp8":
+        raise ValueError(f"kv_dtype {kv_dtype!r}: fp8 or bf16 pools")
     rows = np.empty((n_pages * PAGE, 656), dtype=np.uint8)
     rows[:, :512] = rng.integers(0, 256, size=(n_pages * PAGE, 512), dtype=np.uint8)
     sc = np.exp2(rng.uniform(-20, 4, size=(n_pages * PAGE, 4))).astype(np.float32)

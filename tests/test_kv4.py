@@ -124,3 +124,17 @@ def test_python_refusals(built_lib):
         glmkv.evict_rows(A, A, 1, 1, 1, A, None, None, None, kv_dtype="int8", stream=0)
     with pytest.raises(glmkv.GlmKvError, match="invalid argument"):
         glmkv.kv4_attn(A, A, 0, A, 1, A, A, 1, 64, 1.0, A, A, A, 0, 1, stream=0)
+
+
+@pytest.mark.parametrize("kv_dtype", ["FP4", "nvfp4", "int4", "bfloat16", "", None])
+def test_an_unknown_row_format_is_refused(built_lib, kv_dtype):
+    """The append writes by it: bf16 rows in a 4-bit cache would end 2.8 times as far."""
+    import glmkv
+    from glmkv import workload as W
+
+    with pytest.raises(ValueError, match="kv_dtype"):
+        glmkv.mla_prep_full(A, 2752, A, A, A, A, A, A, A, A, A, A, A, 64, 64, kv_dtype=kv_dtype, stream=0)
+    with pytest.raises(ValueError, match="kv_dtype"):
+        glmkv.mla_prep_shared(A, 2752, A, A, A, A, A, A, A, A, 64, 64, kv_dtype=kv_dtype, stream=0)
+    with pytest.raises(ValueError, match="kv_dtype"):
+        W.random_latent_pages(np.random.default_rng(0), 1, kv_dtype)
