@@ -91,9 +91,13 @@ def _ptr(a, kind, name):
 
 def _here(*tensors):
     """The kernels launch on the current device: a tensor of another one is refused."""
-    devices = {a.get_device() for a in tensors if isinstance(a, torch.Tensor) and a.is_cuda}
-    if devices and devices != {torch.cuda.current_device()}:
-        raise ValueError(f"tensors on cuda:{sorted(devices)}, and the current device is cuda:{torch.cuda.current_device()}")
+    here = None
+    for a in tensors:
+        if isinstance(a, torch.Tensor) and a.is_cuda:
+            if here is None:
+                here = torch.cuda.current_device()
+            if a.get_device() != here:
+                raise ValueError(f"a tensor on cuda:{a.get_device()}, and the current device is cuda:{here}")
 
 
 def _stream(stream):
@@ -123,6 +127,7 @@ def _row_bytes(kv_dtype):
 
 def _prep(kv_dtype, x, lda, g_q, g_kv, rope, pos, slot, kv, idx, ik_w, ik_b, qq, qsf, sf_rows, T, stream):
     _row_bytes(kv_dtype)
+    _here(x, g_q, g_kv, rope, pos, slot, kv, idx, ik_w, ik_b, qq, qsf)
     _lib.call(_PREP[kv_dtype], _ptr(x, "bf16", "x"), int(lda), _ptr(g_q, "bf16", "g_q"), _ptr(g_kv, "bf16", "g_kv"),
               _ptr(rope, "bf16", "rope"), _ptr(pos, "i32", "pos"), _ptr(slot, "i64", "slot"), _ptr(kv, "u8", "kv"),
               _ptr(idx, "u8", "idx"), _ptr(ik_w, "bf16", "ik_w"), _ptr(ik_b, "bf16", "ik_b"), _ptr(qq, "u8", "qq"),

@@ -138,3 +138,37 @@ def test_an_unknown_row_format_is_refused(built_lib, kv_dtype):
         glmkv.mla_prep_shared(A, 2752, A, A, A, A, A, A, A, A, 64, 64, kv_dtype=kv_dtype, stream=0)
     with pytest.raises(ValueError, match="kv_dtype"):
         W.random_latent_pages(np.random.default_rng(0), 1, kv_dtype)
+
+
+class _OnDevice1:
+    """Stands in for torch.Tensor in the bindings' eyes: a contiguous tensor of cuda:1."""
+
+    def __init__(self, dtype):
+        self.dtype, self.is_cuda, self.device = dtype, True, "cuda:1"
+
+    def get_device(self):
+        return 1
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return A
+
+
+@pytest.mark.parametrize("kv_dtype", ["fp8", "bf16", "fp4"])
+@pytest.mark.parametrize("at", range(12))
+def test_the_append_refuses_tensors_of_another_device(built_lib, monkeypatch, kv_dtype, at):
+    import torch
+
+    import glmkv
+    from glmkv import ops
+
+    monkeypatch.setattr(ops.torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(ops.torch, "Tensor", _OnDevice1)
+    b, u, i = torch.bfloat16, torch.uint8, torch.int32
+    names = [b, b, b, b, i, torch.int64, u, u, b, b, u, u]  # x, g_q, g_kv, rope, pos, slot, kv, idx, ik_w, ik_b, qq, qsf
+    t = [A] * 12
+    t[at] = _OnDevice1(names[at])
+    with pytest.raises(ValueError, match="current device"):
+        glmkv.mla_prep_full(t[0], 2752, *t[1:], 64, 64, kv_dtype=kv_dtype, stream=0)
