@@ -100,9 +100,16 @@ def _here(*tensors):
                 raise ValueError(f"a tensor on cuda:{a.get_device()}, and the current device is cuda:{here}")
 
 
+# The current stream's handle without a Stream object: 0.3 us against 3.3. The name is not torch's public one, so
+# a torch that lacks it is asked the public way.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(stream):
-    if stream is None:  # torch.cuda.current_stream().cuda_stream without the Stream object: 0.3 us against 3.3
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    if stream is None:
+        if _raw_stream is None:
+            return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(torch.cuda.current_device())
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream

@@ -172,3 +172,18 @@ def test_the_append_refuses_tensors_of_another_device(built_lib, monkeypatch, kv
     t[at] = _OnDevice1(names[at])
     with pytest.raises(ValueError, match="current device"):
         glmkv.mla_prep_full(t[0], 2752, *t[1:], 64, 64, kv_dtype=kv_dtype, stream=0)
+
+
+def test_the_current_stream_without_torchs_private_name(monkeypatch):
+    from types import SimpleNamespace
+
+    from glmkv import ops
+
+    monkeypatch.setattr(ops.torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(ops.torch.cuda, "current_stream", lambda: SimpleNamespace(cuda_stream=77))
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 100 + device)
+    assert ops._stream(None) == 103
+    monkeypatch.setattr(ops, "_raw_stream", None)
+    monkeypatch.delattr(ops.torch._C, "_cuda_getCurrentRawStream", raising=False)
+    assert ops._stream(None) == 77
+    assert ops._stream(5) == 5 and ops._stream(SimpleNamespace(cuda_stream=6)) == 6
