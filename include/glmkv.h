@@ -62,6 +62,14 @@ enum {
 int glmkv_plan(const int64_t* cu, const int32_t* seq_lens, int nseq, int32_t* pos, uint32_t* ks, uint32_t* ke,
                int32_t* klen, int32_t* row_seq, int32_t* zero, int T, glmkv_stream_t stream);
 
+/* The plan of a call some of whose sequences have lost tokens to an eviction. seen [nseq] i32: the tokens each
+ * sequence has had in all, this call's fresh ones included. pos counts from seen (a token's place in the text: what
+ * its key and its query are roped with), everything else from seq_lens (its place in the cache). Otherwise
+ * as glmkv_plan, and the same where seen is seq_lens. No counterpart in the reference. */
+int glmkv_plan_seen(const int64_t* cu, const int32_t* seq_lens, const int32_t* seen, int nseq, int32_t* pos,
+                    uint32_t* ks, uint32_t* ke, int32_t* klen, int32_t* row_seq, int32_t* zero, int T,
+                    glmkv_stream_t stream);
+
 /* The latent-cache append with the q_a norm + quant, bf16 latent rows (--kv bf16).
  * Replaces ops `mla_prep_full` / `mla_prep_shared` -> glm_mla_prep (kern-glm53 scripts/gen.py:172-177;
  * source/glm_glue.cu:202-296). x [T, lda] bf16: q_a 2048 | kv_a 512 | k_pe 64 | wk 128; rope [pos][64]
@@ -246,7 +254,7 @@ int glmkv_mqa_logits_paged(const void* iq, const void* idx, int n_pages, const i
                            int R, glmkv_stream_t stream);
 
 /* The launch shape (grid x, block x, dynamic shared memory bytes) libglmkv uses for the kernel
- * `entry` ("glm_plan", "glm_mla_prep", "glm_mla_prep_fp8", "glm_idx_gather", "glm_kv_dequant",
+ * `entry` ("glm_plan", "glm_plan_seen", "glm_mla_prep", "glm_mla_prep_fp8", "glm_idx_gather", "glm_kv_dequant",
  * "glm_topk_stream", "glm_topk_slots", "glm_q_post", "glm_add_rms_quant", "glm_mqa_logits_paged",
  * "glm_mark_rows", "glm_topk_stream_mark", "glm_kv_dequant_marked", "glm_mla_prep_fp4", "glm_kv4_dequant",
  * "glm_kv4_attn", "glm_kv4_attn_picks", "glm_kv4_weights") on the current device for a

@@ -206,6 +206,16 @@ GLMKV_API int glmkv_plan(const int64_t* cu, const int32_t* seq_lens, int nseq, i
                 nseq, pos, ks, ke, klen, row_seq, zero, T);
 }
 
+GLMKV_API int glmkv_plan_seen(const int64_t* cu, const int32_t* seq_lens, const int32_t* seen, int nseq, int32_t* pos,
+                              uint32_t* ks, uint32_t* ke, int32_t* klen, int32_t* row_seq, int32_t* zero, int T,
+                              glmkv_stream_t stream) {
+  if (T < 0 || nseq < 1) return GLMKV_ERR_ARG;
+  if (T == 0) return GLMKV_OK;
+  if (!cu || !seq_lens || !seen || !pos || !ks || !ke || !klen || !row_seq || !zero) return GLMKV_ERR_ARG;
+  return launch(glm_plan_seen, (T + PLAN_THREADS - 1) / PLAN_THREADS, PLAN_THREADS, 0, stream, (const long long*)cu,
+                seq_lens, seen, nseq, pos, ks, ke, klen, row_seq, zero, T);
+}
+
 GLMKV_API int glmkv_mla_prep(const void* x, int lda, const void* g_q, const void* g_kv, const void* rope,
                              const int32_t* pos, const int64_t* slot, void* kv, void* idx, const void* ik_w,
                              const void* ik_b, void* qq, void* qsf, int sf_rows, int T, glmkv_stream_t stream) {
@@ -527,7 +537,7 @@ GLMKV_API int glmkv_mqa_logits_paged(const void* iq, const void* idx, int n_page
 GLMKV_API int glmkv_launch_shape(const char* entry, int T, int* grid, int* block, int* smem_bytes) {
   if (!entry || !grid || !block || !smem_bytes || T < 0) return GLMKV_ERR_ARG;
   const auto is = [entry](const char* s) { return strcmp(entry, s) == 0; };
-  if (is("glm_plan")) {
+  if (is("glm_plan") || is("glm_plan_seen")) {
     *grid = (T + PLAN_THREADS - 1) / PLAN_THREADS, *block = PLAN_THREADS, *smem_bytes = 0;
   } else if (is("glm_quant")) {
     return GLMKV_ERR_ARG;  // its grid depends on K too: ceil(T * ceil(K / 512) / 8), block 256

@@ -16,17 +16,14 @@ constexpr uint64_t WAIT_LIMIT_NS = 1000000000ull;  // a bounded wait gives up af
 constexpr int PLAN_THREADS = 256;
 constexpr int PLAN_STAGED = 256;  // sequences whose cu / prefix a block keeps in shared memory
 
-}  // namespace glmkv
-
 // A row's sequence, position and indexer bounds (glm_glue.cu:105-125): s is the first sequence
 // with s + 1 == nseq or cu[s + 1] > r, p = seq_lens[s] - (cu[s + 1] - r), ks the u32 sum of the
-// lengths before s, ke = ks + p + 1, klen = p + 1, row_seq = s, zero = 0.
-//   grid ceil(T / 256), block 256
-extern "C" __global__ void __launch_bounds__(glmkv::PLAN_THREADS)
-    glm_plan(const long long* __restrict__ cu, const int* __restrict__ seq_lens, int nseq, int* __restrict__ pos,
-             unsigned* __restrict__ ks, unsigned* __restrict__ ke, int* __restrict__ klen, int* __restrict__ row_seq,
-             int* __restrict__ zero, int T) {
-  using namespace glmkv;
+// lengths before s, ke = ks + p + 1, klen = p + 1, row_seq = s, zero = 0. pos is p, or, where `seen` is
+// given, seen[s] - (cu[s + 1] - r).
+__device__ __forceinline__ void plan_rows(const long long* __restrict__ cu, const int* __restrict__ seq_lens,
+                                          const int* __restrict__ seen, int nseq, int* __restrict__ pos,
+                                          unsigned* __restrict__ ks, unsigned* __restrict__ ke, int* __restrict__ klen,
+                                          int* __restrict__ row_seq, int* __restrict__ zero, int T) {
   __shared__ long long s_cu[PLAN_STAGED + 1];
   __shared__ unsigned s_off[PLAN_STAGED + 1];
   __shared__ int s_len[PLAN_STAGED];
@@ -60,12 +57,31 @@ extern "C" __global__ void __launch_bounds__(glmkv::PLAN_THREADS)
     len = seq_lens[s];
   }
   const int p = len - (int)(cnext - r);
-  pos[r] = p;
+  pos[r] = seen != nullptr ? seen[s] - (int)(cnext - r) : p;
   ks[r] = goff;
   ke[r] = goff + (unsigned)p + 1u;
   klen[r] = p + 1;
   row_seq[r] = s;
   zero[r] = 0;
+}
+
+}  // namespace glmkv
+
+// The plan of a call whose sequences hold all their tokens.
+//   grid ceil(T / 256), block 256
+extern "C" __global__ void __launch_bounds__(glmkv::PLAN_THREADS)
+    glm_plan(const long long* __restrict__ cu, const int* __restrict__ seq_lens, int nseq, int* __restrict__ pos,
+             unsigned* __restrict__ ks, unsigned* __restrict__ ke, int* __restrict__ klen, int* __restrict__ row_seq,
+             int* __restrict__ zero, int T) {
+  glmkv::plan_rows(cu, seq_lens, nullptr, nseq, pos, ks, ke, klen, row_seq, zero, T);
+}
+// The same where tokens have been evicted: a row's position in the text no longer follows from its sequence's
+// cache length, but from the tokens the sequence has seen. No counterpart in the reference. Same launch.
+extern "C" __global__ void __launch_bounds__(glmkv::PLAN_THREADS)
+    glm_plan_seen(const long long* __restrict__ cu, const int* __restrict__ seq_lens, const int* __restrict__ seen,
+                  int nseq, int* __restrict__ pos, unsigned* __restrict__ ks, unsigned* __restrict__ ke,
+                  int* __restrict__ klen, int* __restrict__ row_seq, int* __restrict__ zero, int T) {
+  glmkv::plan_rows(cu, seq_lens, seen, nseq, pos, ks, ke, klen, row_seq, zero, T);
 }
 
 // ================================================================================================ prep

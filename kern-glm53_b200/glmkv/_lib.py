@@ -13,6 +13,7 @@ CUBIN_PATH = pathlib.Path(__file__).resolve().parent / "glm_glue_b200.cubin"
 P, I, L, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 SIGNATURES = {
     "glmkv_plan": [P, P, I, P, P, P, P, P, P, I, P],
+    "glmkv_plan_seen": [P, P, P, I, P, P, P, P, P, P, I, P],
     "glmkv_mla_prep": [P, I, P, P, P, P, P, P, P, P, P, P, P, I, I, P],
     "glmkv_mla_prep_fp8": [P, I, P, P, P, P, P, P, P, P, P, P, P, I, I, P],
     "glmkv_mla_prep_fp4": [P, I, P, P, P, P, P, P, P, P, P, P, P, I, I, P],

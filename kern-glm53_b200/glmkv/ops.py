@@ -52,6 +52,7 @@ The 4-bit latent cache (416 B a token) has no manifest op. ``mla_prep_*`` append
     evict_plan       acc, pos, n_pages, block_table, max_pages,           glm_evict_plan
                      seq_lens, seen, nseq, budget, sink, recent, moves,
                      n_moves, new_lens: which tokens leave
+    plan             with seen=...: positions after an eviction           glm_plan_seen
     evict_rows       moves, n_moves, nseq, budget, n_pages, kv, idx,      glm_evict_rows*
                      acc, pos: the survivors' moves, any latent format
 
@@ -115,8 +116,13 @@ def _stream(stream):
     return stream.cuda_stream
 
 
-def plan(cu, seq_lens, nseq, pos, ks, ke, klen, row_seq, zero, T, stream=None):
-    _lib.call("glmkv_plan", _ptr(cu, "i64", "cu"), _ptr(seq_lens, "i32", "seq_lens"), int(nseq),
+def plan(cu, seq_lens, nseq, pos, ks, ke, klen, row_seq, zero, T, stream=None, *, seen=None):
+    """Each row's sequence, position and bounds. seen [nseq] i32: the tokens each sequence has had in all, for
+    sequences that evict_plan has cut; pos then counts from it, and all else from seq_lens."""
+    name, lens = "glmkv_plan", (_ptr(seq_lens, "i32", "seq_lens"),)
+    if seen is not None:
+        name, lens = "glmkv_plan_seen", lens + (_ptr(seen, "i32", "seen"),)
+    _lib.call(name, _ptr(cu, "i64", "cu"), *lens, int(nseq),
               _ptr(pos, "i32", "pos"), _ptr(ks, "u32", "ks"), _ptr(ke, "u32", "ke"), _ptr(klen, "i32", "klen"),
               _ptr(row_seq, "i32", "row_seq"), _ptr(zero, "i32", "zero"), int(T), _stream(stream))
 

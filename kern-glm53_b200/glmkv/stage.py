@@ -119,7 +119,8 @@ def forwarded_picks(cut_list):
 
 @dataclass
 class CallMeta:
-    """A call's metadata on the device (gen.py:212-218): cu_seqlens, seq_lens, block_table, slot_mapping."""
+    """A call's metadata on the device (gen.py:212-218): cu_seqlens, seq_lens, block_table, slot_mapping. `seen`
+    [nseq] i32 where an eviction has cut sequences: the tokens each has had in all, the call's own included."""
     cu: torch.Tensor
     seq_lens: torch.Tensor
     block_table: torch.Tensor
@@ -127,6 +128,7 @@ class CallMeta:
     nseq: int
     T: int
     ctx: int
+    seen: torch.Tensor = None
 
     @property
     def max_pages(self):
@@ -188,7 +190,7 @@ class LayerGroup:
         hook = on_op or (lambda op, l, before: None)
         hook("plan", None, True)
         ops.plan(meta.cu, meta.seq_lens, nseq, self.pos, self.ks, self.ke, self.klen, self.row_seq, self.zero, T,
-                 stream=stream)
+                 stream=stream, seen=meta.seen)
         hook("plan", None, False)
         for l in self.layers:
             a = inputs[l]

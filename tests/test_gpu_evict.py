@@ -200,3 +200,112 @@ def test_a_serving_loop(cuda):
             lens[s] = stay.sum()
         assert np.array_equal(dl.cpu().numpy(), lens)
     assert glmkv.fault_flags() == 0
+
+
+@pytest.mark.parametrize("nseq", [1, 3, 257, 700])
+def test_plan_takes_positions_from_what_was_seen(cuda, nseq):
+    import glmkv
+
+    rng = np.random.default_rng(nseq)
+    fresh = rng.integers(0, 6, nseq)
+    fresh[-1] += 1
+    lens = fresh + rng.integers(0, 200, nseq)
+    seen = lens + rng.integers(0, 1000, nseq)
+    cu = np.concatenate([[0], np.cumsum(fresh)])
+    T = int(cu[-1])
+    g = lambda a, dt=np.int32: torch.from_numpy(np.asarray(a).astype(dt)).to(cuda)
+    outs = []
+    for kw in ({}, {"seen": g(seen)}, {"seen": g(lens)}):
+        o = [torch.full((T,), -7, dtype=torch.int32, device=cuda) for _ in range(6)]
+        glmkv.plan(g(cu, np.int64), g(lens), nseq, *o, T, **kw)
+        outs.append([v.cpu().numpy() for v in o])
+    seq = np.repeat(np.arange(nseq), fresh)
+    behind = cu[seq + 1] - np.arange(T)  # a row's distance from its sequence's end
+    assert np.array_equal(outs[0][0], lens[seq] - behind) and np.array_equal(outs[1][0], seen[seq] - behind)
+    for a, b in zip(outs[0][1:], outs[1][1:]):
+        assert np.array_equal(a, b)
+    for a, b in zip(outs[0], outs[2]):
+        assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("kv_dtype", ["fp4", "fp8", "bf16"])
+def test_a_stage_goes_on_after_an_eviction(cuda, kv_dtype):
+    """Two calls of a stage, its sequences cut between them, beside a stage whose are not: the second call's rows and
+    indexer keys are the same bytes in both, whatever the sequences still hold."""
+    import glmkv
+    from glmkv import stage, workload as W
+    from oracle import kv4
+
+    rng = np.random.default_rng(17)
+    nseq, max_pages, n_pages, budget, sink, recent = 3, 7, 23, 150, 4, 32
+    row = {"fp4": 416, "fp8": 656, "bf16": 1152}[kv_dtype]
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda)
+    bf = lambda a: t(a.view(np.int16)).view(torch.bfloat16)
+    bt = rng.permutation(n_pages)[:nseq * max_pages].reshape(nseq, max_pages).astype(np.int32)
+    rope = bf(W.rope_table(1024))
+    weights = {l: W.weights(rng) for l in range(4)}
+    groups = {}
+    for name in ("cut", "whole"):
+        g = groups[name] = stage.LayerGroup(0, 4, n_pages=n_pages, max_ctx=nseq * max_pages * 64, chunk=512,
+                                            kv_dtype=kv_dtype, device=cuda)
+        g.rope = rope
+        for v in [*g.kv.values(), *g.idx.values()]:
+            v.zero_()
+    lens = {name: np.zeros(nseq, np.int32) for name in groups}
+    seen = np.zeros(nseq, np.int32)
+    acc = t(rng.random(n_pages * 64).astype(np.float32))
+    pos = torch.zeros(n_pages * 64, dtype=torch.int32, device=cuda)
+    new = {}
+    for step, fresh in enumerate([[300, 100, 64], [3, 90, 1]]):
+        fresh = np.array(fresh, np.int32)
+        T = int(fresh.sum())
+        seq, rel = np.repeat(np.arange(nseq), fresh), np.concatenate([np.arange(f) for f in fresh])
+        cu = np.concatenate([[0], np.cumsum(fresh)]).astype(np.int64)
+        x = {l: bf(W.activations(rng, T)) for l in range(4)}
+        seen = seen + fresh
+        for name, g in groups.items():
+            at = lens[name][seq] + rel
+            slot = bt[seq, at // 64].astype(np.int64) * 64 + at % 64
+            lens[name] = lens[name] + fresh
+            inputs = {l: stage.LayerInputs(x[l], bf(w.g_q), bf(w.g_kv), *((bf(w.ik_w), bf(w.ik_b)) if l in stage.FULL
+                                                                         else ())) for l, w in weights.items()}
+            ind = {l: torch.arange(2048, dtype=torch.int32, device=cuda).repeat(T, 1) for l in range(3)}
+            meta = stage.CallMeta(t(cu), t(lens[name]), t(bt), t(slot), nseq, T, int(lens[name].sum()),
+                                  seen=t(seen) if name == "cut" else None)
+            g.run_call(meta, inputs, ind)
+            torch.cuda.synchronize()
+            new[name] = slot
+            assert np.array_equal(g.pos[:T].cpu().numpy(), (seen[seq] - fresh[seq]) + rel)
+            if name == "cut":
+                pos[t(slot)] = g.pos[:T]
+        rows = {n: {l: g.kv[l].cpu().numpy().reshape(-1, row) for l in g.kv} for n, g in groups.items()}
+        keys = {n: {l: g.idx[l].cpu().numpy().reshape(n_pages, 8448) for l in g.idx} for n, g in groups.items()}
+        key = lambda pool, s: (pool[s // 64, :8192].reshape(len(s), 64, 128)[np.arange(len(s)), s % 64],
+                               pool[s // 64, 8192:].reshape(len(s), 64, 4)[np.arange(len(s)), s % 64])
+        for l in range(4):
+            assert np.array_equal(rows["cut"][l][new["cut"]], rows["whole"][l][new["whole"]]), (step, l)
+        for l in range(3):
+            for a, b in zip(key(keys["cut"][l], new["cut"]), key(keys["whole"][l], new["whole"])):
+                assert np.array_equal(a, b), (step, l)
+        if step == 0:
+            g = groups["cut"]
+            dl = t(lens["cut"])
+            moves = torch.zeros(nseq, budget, 2, dtype=torch.int32, device=cuda)
+            n_moves = torch.zeros(nseq, dtype=torch.int32, device=cuda)
+            glmkv.evict_plan(acc, pos, n_pages, t(bt), max_pages, dl, t(seen), nseq, budget, sink, recent, moves, n_moves,
+                             dl)
+            for l in g.kv:
+                glmkv.evict_rows(moves, n_moves, nseq, budget, n_pages, g.kv[l], g.idx.get(l), None, None,
+                                 kv_dtype=kv_dtype)
+            glmkv.evict_rows(moves, n_moves, nseq, budget, n_pages, None, None, acc, pos)
+            torch.cuda.synchronize()
+            lens["cut"] = dl.cpu().numpy()
+            assert lens["cut"].tolist() == [150, 100, 64]
+    # every survivor is the row of its position in the stage that lost none
+    where = pos.cpu().numpy()
+    for s in range(nseq):
+        at = kv4.slots_of(bt, s, int(lens["cut"][s]))
+        src = kv4.slots_of(bt, s, int(lens["whole"][s]))[where[at]]
+        for l in range(4):
+            assert np.array_equal(rows["cut"][l][at], rows["whole"][l][src])
+    assert glmkv.fault_flags() == 0

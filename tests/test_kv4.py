@@ -187,3 +187,21 @@ def test_the_current_stream_without_torchs_private_name(monkeypatch):
     monkeypatch.delattr(ops.torch._C, "_cuda_getCurrentRawStream", raising=False)
     assert ops._stream(None) == 77
     assert ops._stream(5) == 5 and ops._stream(SimpleNamespace(cuda_stream=6)) == 6
+
+
+def test_plan_with_seen_checks_its_arguments(built_lib):
+    import torch
+
+    import glmkv
+    from glmkv import _lib
+
+    fn = glmkv.lib().glmkv_plan_seen
+    good = [A, A, A, 2, A, A, A, A, A, A, 16, None]  # cu, seq_lens, seen, nseq, outputs, T, stream
+    for i, v in [(3, 0), (10, -1)] + [(i, None) for i in (0, 1, 2, 4, 5, 6, 7, 8, 9)]:
+        assert fn(*[v if j == i else a for j, a in enumerate(good)]) == _lib.ERR_ARG, (i, v)
+    assert fn(*[0 if j == 10 else a for j, a in enumerate(good)]) == _lib.OK
+    if not torch.cuda.is_available():
+        with pytest.raises(glmkv.GlmKvError, match="glmkv_plan:"):
+            glmkv.plan(A, A, 2, A, A, A, A, A, A, 16, stream=0)
+        with pytest.raises(glmkv.GlmKvError, match="glmkv_plan_seen:"):
+            glmkv.plan(A, A, 2, A, A, A, A, A, A, 16, stream=0, seen=A)
