@@ -715,6 +715,10 @@ __device__ __forceinline__ void a4_run(const A4Args& a) {
           float p[32];
           auto weigh = [&]() {
             float mx = -INFINITY;
+            // -0, which the compiler does not know (heads <= 1024): a product as an fma with it. A packed multiply
+            // with a packed add behind it comes out fused (one rounding, measured), although both say .rn.
+            const float z = __uint_as_float(0x80000000u + ((uint32_t)a.heads >> 11));
+            const float2 mz = make_float2(z, z);
 #pragma unroll
             for (int j = 0; j < 32; j += 16) {
               if (r0 + j >= nrows) {
@@ -730,10 +734,12 @@ __device__ __forceinline__ void a4_run(const A4Args& a) {
               for (int i = 0; i < 16; i += 4) {
                 const float4 f4 = *reinterpret_cast<const float4*>(f + j + i);
                 const float4 n4 = *reinterpret_cast<const float4*>(nm + r0 + j + i);
-                const float2 lo = fma2(make_float2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])),
-                                       make_float2(f4.x, f4.y), make_float2(n4.x, n4.y));
-                const float2 hi = fma2(make_float2(__uint_as_float(u[i + 2]), __uint_as_float(u[i + 3])),
-                                       make_float2(f4.z, f4.w), make_float2(n4.z, n4.w));
+                // The score is rounded before the reference is taken off, as in the maximum that set it: past 2^28
+                // that rounding is more than a weight's exponent has room for, and a fused difference would show it.
+                const float2 lo = add2(fma2(make_float2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])),
+                                            make_float2(f4.x, f4.y), mz), make_float2(n4.x, n4.y));
+                const float2 hi = add2(fma2(make_float2(__uint_as_float(u[i + 2]), __uint_as_float(u[i + 3])),
+                                            make_float2(f4.z, f4.w), mz), make_float2(n4.z, n4.w));
                 x[i] = lo.x, x[i + 1] = lo.y, x[i + 2] = hi.x, x[i + 3] = hi.y;
               }
               if (masked) {

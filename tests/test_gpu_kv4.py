@@ -130,6 +130,47 @@ def test_attention_of_sharp_flat_and_scaled_rows(cuda, q_std, scale):
     c.check_attn(_np(d["out"]), _np(d["lse"]))
 
 
+def _check_far(c, d):
+    """Scores so large that their rounding in f32 is many powers of two: a row whose largest one leads by more than
+    twice the scores' error and 40 more has that token's latents, which bf16 holds exactly, and its score for lse. A
+    score's error: a sum of 576 products in f32, twice that with a truncating adder, and its factors' roundings. The
+    tokens behind weigh 2^-57 each or less, and the output is off by its own rounding and the reciprocal's, together
+    below 2^-8. lse is off by the score's error and two roundings."""
+    from oracle import kv4
+
+    out, lse = _np(d["out"]).astype(np.float64), _np(d["lse"]).astype(np.float64)
+    assert np.all(np.isfinite(out)) and np.all(np.isfinite(lse))
+    sure = 0
+    for t in range(c.T):
+        lat, pe = kv4.lift(c.kv[c.rows_of(t)])
+        k = np.concatenate([lat, pe], 1)
+        x = c.scale * (c.q[t] @ k.T)
+        ds = (abs(c.scale) * (np.abs(c.q[t]) @ np.abs(k).T)).max(1) * 578 * 2.0 ** -23
+        first, second = np.sort(x, 1)[:, -1], np.sort(x, 1)[:, -2]
+        lead = first - second > 2 * ds + 40
+        sure += lead.sum()
+        want = lat[x.argmax(1)]
+        assert np.all((np.abs(out[t] - want) <= np.abs(want) * 2.0 ** -8 + 2.0 ** -40)[lead])
+        assert np.all((np.abs(lse[t] - first) <= ds + np.abs(first) * 2.0 ** -22)[lead])
+    assert sure > 0.9 * c.T * c.heads
+
+
+FAR = [(3e6, [200, 90], [2, 1]), (3e7, [200, 90], [2, 1]), (1e9, [1500, 77], [2, 1]), (-1e12, [1500, 77], [2, 1]),
+       (1e30, [300, 129], [1, 1]), (1e9, [20000], [1])]
+
+
+@pytest.mark.parametrize("scale,lens,qlens", FAR)
+def test_attention_of_far_scores(cuda, scale, lens, qlens):
+    """A reference past 2^28 is rounded by more than a weight's exponent has room for."""
+    from kv4_case import Kv4Case
+
+    c = Kv4Case(lens, qlens, 64, seed=13)
+    c.scale = scale
+    d = c.device(torch, cuda)
+    c.attn(d)
+    _check_far(c, d)
+
+
 def test_attention_rising_scores(cuda):
     """Every tile's scores pass the last one's: the rows are rescaled a tile."""
     from kv4_case import Kv4Case, bf16
