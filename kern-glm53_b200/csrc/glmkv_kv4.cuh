@@ -58,7 +58,7 @@ constexpr int A4_SMEM = 1024 + A4_BLOCKS * (A4_KBLK + A4_QBLK);  // 222,208 B wi
 constexpr int A4_TMEM = 512, A4_O = 0, A4_S = 256;   // O^T: four 64-column blocks; S^T: two buffers of 64
 constexpr int A4_NONE = INT_MIN;
 constexpr int A4_NAN = INT_MIN;                      // set in the slot of a token that has a NaN scale
-constexpr float A4_LOW = -1e30f;                     // a row's reference before its first token
+constexpr float A4_LOW = -3.402823466e38f;           // a row's reference before its first token: no score is lower
 constexpr float A4_OFF = 7.f, A4_TOP = 15.f;         // P = 2^(s - m + 7); m is raised past 2^15
 // part of a split item: O^T as [64 rows][512] f32, then 64 references and 64 sums; two a CTA
 constexpr int A4_PART = A4_ROWS * (KVL + 2) * 4;

@@ -171,6 +171,23 @@ def test_attention_of_far_scores(cuda, scale, lens, qlens):
     _check_far(c, d)
 
 
+@pytest.mark.parametrize("scale", [1e9, 1e29])
+@pytest.mark.parametrize("n", [100, 300, 20000])
+def test_attention_of_scores_far_below_zero(cuda, scale, n):
+    """Every score of a row below the reference that a row starts with, in a first tile and in later ones."""
+    from kv4_case import Kv4Case, bf16
+    from oracle import kv4
+
+    c = Kv4Case([n], [1], 48, seed=14)
+    lat, pe = bf16(np.abs(c.rng.standard_normal((n, 512)))), bf16(np.abs(c.rng.standard_normal((n, 64))))
+    c.kv[kv4.slots_of(c.bt, 0, n)] = kv4.pack(lat[1], pe[0])
+    c.q_bits, c.q = bf16(-np.abs(c.rng.standard_normal(c.q.shape)))
+    c.scale = scale
+    d = c.device(torch, cuda)
+    c.attn(d)
+    _check_far(c, d)
+
+
 def test_attention_rising_scores(cuda):
     """Every tile's scores pass the last one's: the rows are rescaled a tile."""
     from kv4_case import Kv4Case, bf16
