@@ -257,10 +257,12 @@ int glmkv_mqa_logits_paged(const void* iq, const void* idx, int n_pages, const i
  * `entry` ("glm_plan", "glm_plan_seen", "glm_mla_prep", "glm_mla_prep_fp8", "glm_idx_gather", "glm_kv_dequant",
  * "glm_topk_stream", "glm_topk_slots", "glm_q_post", "glm_add_rms_quant", "glm_mqa_logits_paged",
  * "glm_mark_rows", "glm_topk_stream_mark", "glm_kv_dequant_marked", "glm_mla_prep_fp4", "glm_kv4_dequant",
- * "glm_kv4_attn", "glm_kv4_attn_picks", "glm_kv4_weights") on the current device for a
- * call of T fresh rows: what a kern
- * manifest's `impl.launches` entry for the cubin must use. The persistent page kernels depend on the
- * device's SM count only. No counterpart in the reference, whose shapes are fixed in its manifest
+ * "glm_kv4_attn", "glm_kv4_attn_picks", "glm_kv4_weights", "glm_kv4_join") on the current device for a
+ * call of T fresh rows: what a kern manifest's `impl.launches` entry for the cubin must use. The persistent page
+ * kernels depend on the device's SM count only. glm_kv4_attn and glm_kv4_attn_picks are always followed by
+ * glm_kv4_join, whose G is their grid: it writes the rows that several CTAs shared. The eviction's kernels are for the
+ * library's launchers alone (GLMKV_ERR_ARG here): a plan's cluster, and how many keys fit its shared memory, follow
+ * from the whole call. No counterpart in the reference, whose shapes are fixed in its manifest
  * generator (kern-glm53 scripts/gen.py:95-135, 172-177). */
 int glmkv_launch_shape(const char* entry, int T, int* grid, int* block, int* smem_bytes);
 

@@ -559,7 +559,7 @@ GLMKV_API int glmkv_launch_shape(const char* entry, int T, int* grid, int* block
     *grid = std::min(d->sms, std::max(1, (T + MK_RB - 1) / MK_RB)), *block = MK_THREADS, *smem_bytes = MK_SMEM;
   } else if (is("glm_kv_dequant") || is("glm_kv_dequant_marked") || is("glm_idx_gather") || is("glm_mla_prep") ||
              is("glm_mla_prep_fp8") || is("glm_mla_prep_fp4") || is("glm_kv4_dequant") || is("glm_kv4_attn") ||
-             is("glm_kv4_attn_picks") || is("glm_kv4_weights")) {
+             is("glm_kv4_attn_picks") || is("glm_kv4_weights") || is("glm_kv4_join")) {
     const DeviceInfo* d = device_info();
     if (!d) return GLMKV_ERR_DEVICE;
     if (is("glm_kv_dequant") || is("glm_kv_dequant_marked")) {
@@ -568,6 +568,8 @@ GLMKV_API int glmkv_launch_shape(const char* entry, int T, int* grid, int* block
       *grid = d->sms, *block = DQ_THREADS, *smem_bytes = (int)D4_SMEM;
     } else if (is("glm_kv4_attn") || is("glm_kv4_attn_picks") || is("glm_kv4_weights")) {
       *grid = d->sms, *block = A4_THREADS, *smem_bytes = A4_SMEM;
+    } else if (is("glm_kv4_join")) {
+      *grid = 2 * d->sms, *block = J4_THREADS, *smem_bytes = 0;
     } else if (is("glm_idx_gather")) {
       *grid = d->sms * d->ga_ctas, *block = GA_THREADS, *smem_bytes = (int)GA_SMEM;
     } else {

@@ -205,3 +205,24 @@ def test_plan_with_seen_checks_its_arguments(built_lib):
             glmkv.plan(A, A, 2, A, A, A, A, A, A, 16, stream=0)
         with pytest.raises(glmkv.GlmKvError, match="glmkv_plan_seen:"):
             glmkv.plan(A, A, 2, A, A, A, A, A, A, 16, stream=0, seen=A)
+
+
+def test_launch_shapes_known_to_the_library(built_lib):
+    """Every kernel that a cubin's user may launch has a shape (without a device: the query for it is reached); the
+    eviction's, whose clusters follow from the call, are refused."""
+    import torch
+
+    import glmkv
+
+    names = ["glm_mla_prep_fp4", "glm_kv4_dequant", "glm_kv4_attn", "glm_kv4_attn_picks", "glm_kv4_weights", "glm_kv4_join"]
+    for name in names:
+        if torch.cuda.is_available():
+            assert min(glmkv.launch_shape(name, 8)[:2]) > 0
+        else:
+            with pytest.raises(glmkv.GlmKvError) as e:
+                glmkv.launch_shape(name, 8)
+            assert e.value.code == glmkv._lib.ERR_DEVICE, name
+    assert glmkv.launch_shape("glm_plan_seen", 600) == glmkv.launch_shape("glm_plan", 600) == (3, 256, 0)
+    for name in ("glm_evict_plan", "glm_evict_rows", "glm_evict_rows_fp4", "glm_evict_rows_fp8"):
+        with pytest.raises(glmkv.GlmKvError, match="invalid argument"):
+            glmkv.launch_shape(name, 8)
