@@ -16,6 +16,12 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: long CPU test")
 
 
+def pytest_collection_modifyitems(items):
+    """The tests that need the reference's own kernels come last: where its library is not there they fail, and a run
+    that ends at its first failure has then run all the others."""
+    items.sort(key=lambda item: "ref" in getattr(item, "fixturenames", ()))
+
+
 @pytest.fixture(scope="session")
 def built_lib():
     """libglmkv.so, (re)built in-tree when stale (nvcc cross-compiles; no GPU needed)."""
