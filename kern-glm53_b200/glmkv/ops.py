@@ -92,13 +92,15 @@ def _ptr(a, kind, name):
 
 def _here(*tensors):
     """The kernels launch on the current device: a tensor of another one is refused."""
-    here = None
+    here = -1
     for a in tensors:
-        if isinstance(a, torch.Tensor) and a.is_cuda:
-            if here is None:
-                here = torch.cuda.current_device()
-            if a.get_device() != here:
-                raise ValueError(f"a tensor on cuda:{a.get_device()}, and the current device is cuda:{here}")
+        if isinstance(a, torch.Tensor):
+            device = a.get_device()  # -1: not a GPU's, which _ptr refuses
+            if device >= 0 and device != here:
+                if here < 0:
+                    here = torch.cuda.current_device()
+                if device != here:
+                    raise ValueError(f"a tensor on cuda:{device}, and the current device is cuda:{here}")
 
 
 # The current stream's handle without a Stream object: 0.3 us against 3.3. The name is not torch's public one, so
