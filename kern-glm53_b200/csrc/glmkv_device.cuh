@@ -130,8 +130,9 @@ __device__ __forceinline__ uint32_t dequant2(uint16_t pair, float sc) {
 
 // The 4-bit latent row: 16 values share an e4m3 scale s = e4m3(amax / 6), so the largest lands near 6,
 // e2m1's largest. A value's code is e2m1(v / s), round to nearest even, saturating; 0 where s is 0
-// (amax below 6 * 2^-10). e2m1 has 2 significant bits and e4m3 4, so a lifted value, code * s, has at
-// most 6 and lies in [2^-10, 2688]: exact in bf16 and in f16.
+// (amax below 6 * 2^-10). s is NaN where one of the 16 values is, 448 where one is infinite. e2m1 has 2
+// significant bits and e4m3 4, so a lifted value, code * s, has at most 6 and lies in [2^-10, 2688]: exact in
+// bf16 and in f16.
 __device__ __forceinline__ u8 kv4_scale(float amax) {
   return __nv_cvt_float_to_fp8(__fdiv_rn(amax, 6.f), __NV_SATFINITE, __NV_E4M3);
 }

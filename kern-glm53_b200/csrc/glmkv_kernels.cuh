@@ -129,6 +129,12 @@ __device__ __forceinline__ uint32_t absmax_xs(uint32_t a, uint32_t b) {
   asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// The same, NaN where either operand is.
+__device__ __forceinline__ uint32_t absmax_xs_nan(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 // bf16x2 add and multiply, each half rounded once from the exact result (sm_90+).
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -327,15 +333,17 @@ __device__ __forceinline__ void prep_row(const Row& row, const float* __restrict
     // Groups of 16 columns: the pairs of lanes 8k .. 8k + 7 of virtual warp w are group 4w + k. |max| of
     // virtual warps 2j (low half) and 2j + 1 (high), then a reduce-scatter over the eight lanes leaves
     // lane l with virtual warp l & 7: one group a lane, so the 32 scales are computed at once.
+    // A NaN among the 16 makes the scale NaN, and with it the group: its own code could not say so.
     uint32_t m4[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      m4[j] = absmax_xs(__byte_perm(kn[2 * j], kn[2 * j + 1], 0x5410), __byte_perm(kn[2 * j], kn[2 * j + 1], 0x7632));
+      m4[j] = absmax_xs_nan(__byte_perm(kn[2 * j], kn[2 * j + 1], 0x5410),
+                            __byte_perm(kn[2 * j], kn[2 * j + 1], 0x7632));
     const bool b2 = l & 4, b1 = l & 2;
-    const uint32_t a0 = absmax_xs(b2 ? m4[2] : m4[0], __shfl_xor_sync(FULL, b2 ? m4[0] : m4[2], 4));
-    const uint32_t a1 = absmax_xs(b2 ? m4[3] : m4[1], __shfl_xor_sync(FULL, b2 ? m4[1] : m4[3], 4));
-    uint32_t m = absmax_xs(b1 ? a1 : a0, __shfl_xor_sync(FULL, b1 ? a0 : a1, 2));
-    m = absmax_xs(m, __shfl_xor_sync(FULL, m, 1));
+    const uint32_t a0 = absmax_xs_nan(b2 ? m4[2] : m4[0], __shfl_xor_sync(FULL, b2 ? m4[0] : m4[2], 4));
+    const uint32_t a1 = absmax_xs_nan(b2 ? m4[3] : m4[1], __shfl_xor_sync(FULL, b2 ? m4[1] : m4[3], 4));
+    uint32_t m = absmax_xs_nan(b1 ? a1 : a0, __shfl_xor_sync(FULL, b1 ? a0 : a1, 2));
+    m = absmax_xs_nan(m, __shfl_xor_sync(FULL, m, 1));
     const float gm = __uint_as_float(((l & 1) ? (m & 0xffff0000u) : (m << 16)) & 0x7fffffffu);
     const u8 sb = kv4_scale(gm);
     const float sc = e4m3_value(sb);

@@ -579,7 +579,7 @@ __device__ __forceinline__ void a4_run(const A4Args& a) {
         pe[h] = ks < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(a.kv + (size_t)ks * KV4 + KV4_PE) + (l & 7));
       }
       if constexpr (MODE == A4_ATTN) {
-        // A NaN scale (of a token whose latents were not finite) would reach rows that do not see the token, as
+        // A NaN scale (the append gives a group one that has a NaN latent) would reach rows that do not see the token, as
         // 0 * NaN: it is lifted as zeros, and the token's scores are made NaN instead.
         uint32_t bad = 0;
 #pragma unroll

@@ -67,6 +67,53 @@ def test_append_is_the_packed_bf16_row(cuda, T, full, lda, offset):
     assert len(bad) == 0, f"{len(bad)} bytes differ, first at {bad[:4].tolist()}"
 
 
+@pytest.mark.parametrize("last", [1.0, float("inf"), float("nan")])
+def test_append_over_the_formats_range(cuda, last):
+    """Gains from 2^-16 to 2^14, 16 columns each: groups that become zeros, scales of fewer than four bits, scales that
+    saturate; one infinite or NaN latent, and a row with an infinite input. The row is the packed bf16 row throughout."""
+    import glmkv
+    from glmkv import workload as W
+    from oracle import kv4
+
+    rng = np.random.default_rng(8)
+    T, n_pages = 50, 1
+    w = W.weights(rng)
+    gains = np.repeat(np.exp2(np.arange(32) - 16.0), 16).astype(np.float32)
+    gains[31 * 16:] = 1.0
+    gains[511] = last
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda)
+    b = lambda a: t(a.view(np.int16)).view(torch.bfloat16)
+    xf = rng.standard_normal((T, 2624)).astype(np.float32)
+    xf[3, 2048 + 100] = np.inf                          # the norm's factor is 0, this latent 0 * inf
+    x = W.bf16_bits(xf)
+    got = {}
+    for kv_dtype, row in (("fp4", 416), ("bf16", 1152)):
+        kv = torch.full((n_pages * 64, row), 0xA5, dtype=torch.uint8, device=cuda)
+        qq, qsf = (torch.zeros(n, dtype=torch.uint8, device=cuda) for n in (T * 2048, 16 * T))
+        glmkv.mla_prep_shared(b(x), 2624, b(w.g_q), b(W.bf16_bits(gains)), b(W.rope_table(64)),
+                              torch.zeros(T, dtype=torch.int32, device=cuda), torch.arange(T, device=cuda), kv, qq, qsf, T,
+                              T, kv_dtype=kv_dtype)
+        torch.cuda.synchronize()
+        got[kv_dtype] = kv.cpu().numpy()[:T]
+    assert glmkv.fault_flags() == 0
+    rows, bits = got["fp4"], got["bf16"].copy().view(np.uint16)
+    v = kv4.bf16_value(bits[:, :512])
+    # a group with a NaN is NaN as a whole, by its scale; its codes say nothing
+    nan = np.isnan(v).reshape(T, 32, 16).any(-1)
+    assert nan[3].any() and nan[:, 31].all() == np.isnan(last)
+    assert np.array_equal((rows[:, 256:288] & 0x7F) == 0x7F, nan)
+    v[np.repeat(nan, 16, 1)] = 0
+    rows[:, 256:288][nan], rows[:, :256][np.repeat(nan, 8, 1)] = 0, 0
+    want = kv4.pack(v, bits[:, 512:])
+    assert np.array_equal(rows, want)
+    lat = kv4.lift(rows)[0]
+    top = np.abs(v.reshape(T, 32, 16)).max(-1)
+    assert not lat.reshape(T, 32, 16)[top < 6 * 2.0 ** -10].any() and (top < 6 * 2.0 ** -10).any()
+    if np.isinf(last):
+        rest = np.arange(T) != 3
+        assert np.array_equal(lat[rest, 511], np.sign(v[rest, 511]) * 2688)
+
+
 @pytest.mark.parametrize("lens", [[1], [63, 0, 64, 65, 1], [700, 1, 129, 4000], [0, 0]])
 def test_lift_is_exact(cuda, lens):
     import glmkv
