@@ -309,3 +309,71 @@ def test_a_stage_goes_on_after_an_eviction(cuda, kv_dtype):
         for l in range(4):
             assert np.array_equal(rows["cut"][l][at], rows["whole"][l][src])
     assert glmkv.fault_flags() == 0
+
+
+def test_a_captured_step(cuda):
+    """A whole step in one graph (plan, append, attention, weights, eviction), replayed from a fresh state: what the
+    same calls outside a graph leave."""
+    import glmkv
+    from glmkv import workload as W
+    from kv4_case import bf16
+
+    rng = np.random.default_rng(23)
+    H, nseq, max_pages, n_pages, budget, sink, recent = 16, 20, 3, 64, 70, 4, 16
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda)
+    b = lambda a: t(a.view(np.int16)).view(torch.bfloat16)
+    lens = rng.integers(1, 160, nseq).astype(np.int32)
+    fresh = np.minimum(lens, rng.integers(1, 4, nseq)).astype(np.int32)
+    T = int(fresh.sum())
+    bt = rng.permutation(n_pages)[:nseq * max_pages].reshape(nseq, max_pages).astype(np.int32)
+    seq, rel = np.repeat(np.arange(nseq), fresh), np.concatenate([np.arange(f) for f in fresh])
+    at = (lens - fresh)[seq] + rel
+    slot = t(bt[seq, at // 64].astype(np.int64) * 64 + at % 64)
+    w, x = W.weights(rng), b(W.activations(rng, T))
+    g_q, g_kv, rope, dbt = b(w.g_q), b(w.g_kv), b(W.rope_table(4096)), t(bt)
+    cu = t(np.concatenate([[0], np.cumsum(fresh)]).astype(np.int64))
+    q = b(bf16(rng.standard_normal((T, H, 576)))[0])
+    pos0 = np.zeros(n_pages * 64, np.int32)
+    for s in range(nseq):
+        j = np.arange(lens[s])
+        pos0[bt[s, j // 64] * 64 + j % 64] = 10 * j
+    start = {"kv": torch.randint(0, 120, (n_pages * 64, 416), dtype=torch.uint8, device=cuda), "pos": t(pos0),
+             "acc": torch.rand(n_pages * 64, device=cuda), "lens": t(lens), "seen": t(10 * lens)}
+    start["kv"][:, 256:288] = 0x38                     # scales of 1
+    start["kv"][:, 288:] = 0
+    d = {k: v.clone() for k, v in start.items()}
+    o = {k: torch.zeros(T, dtype=torch.int32, device=cuda) for k in ("p", "ks", "ke", "klen", "row_seq", "zero")}
+    qq, qsf = (torch.zeros(n, dtype=torch.uint8, device=cuda) for n in (T * 2048, 16 * T))
+    out, lse = torch.zeros(T, H, 512, dtype=torch.bfloat16, device=cuda), torch.zeros(T, H, device=cuda)
+    n_ws = glmkv.kv4_workspace_bytes()
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=cuda)
+    moves, n_moves = (torch.zeros(n, dtype=torch.int32, device=cuda) for n in ((nseq, budget, 2), (nseq,)))
+
+    def step():
+        glmkv.plan(cu, d["lens"], nseq, *o.values(), T, seen=d["seen"])
+        glmkv.mla_prep_shared(x, x.shape[1], g_q, g_kv, rope, o["p"], slot, d["kv"], qq, qsf, T, T, kv_dtype="fp4")
+        d["pos"][slot] = o["p"]
+        glmkv.kv4_attn(q, d["kv"], n_pages, dbt, max_pages, cu, d["lens"], nseq, H, 0.0625, out, lse, ws, n_ws, T)
+        glmkv.kv4_weights(q, lse, d["kv"], n_pages, dbt, max_pages, cu, d["lens"], nseq, H, 0.0625, d["acc"], T)
+        glmkv.evict_plan(d["acc"], d["pos"], n_pages, dbt, max_pages, d["lens"], d["seen"], nseq, budget, sink, recent, moves,
+                         n_moves, d["lens"])
+        glmkv.evict_rows(moves, n_moves, nseq, budget, n_pages, d["kv"], None, d["acc"], d["pos"])
+
+    def results():
+        torch.cuda.synchronize()
+        return [v.clone() for v in (*d.values(), *o.values(), out, lse, n_moves)]
+
+    step()
+    want = results()
+    assert int(n_moves.sum()) > 0 and int(want[3].max()) == budget
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        for k, v in start.items():
+            d[k].copy_(v)
+        out.zero_(), lse.zero_()
+        graph.replay()
+        for a, e in zip(results(), want):
+            assert torch.equal(a, e)
+    assert glmkv.fault_flags() == 0

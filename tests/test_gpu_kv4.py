@@ -445,6 +445,67 @@ def test_streams_and_graphs(cuda):
     assert np.all(np.abs(_np(acc) - 2 * want) <= 2 * tol + want * 2.0 ** -22)
 
 
+def test_offsets_past_32_bits(cuda):
+    """A pool of 4.5 GB with the sequences in its last pages: append, lift, attention, picks, weights and moves."""
+    import glmkv
+    from glmkv import workload as W
+    from kv4_case import Kv4Case
+    from oracle import kv4
+
+    c = Kv4Case([500, 130], [2, 1], 16, seed=21)
+    d = c.device(torch, cuda)
+    n_pages = 170000
+    shift = n_pages - c.n_pages
+    kv = torch.empty(n_pages * 64, 416, dtype=torch.uint8, device=cuda)
+    kv[shift * 64:] = d["kv"]
+    d["kv"], c.n_pages = kv, n_pages
+    d["bt"] = torch.where(d["bt"] >= 0, d["bt"] + shift, d["bt"])
+    c.bt = np.where(c.bt >= 0, c.bt + shift, c.bt)
+    small, c.kv = c.kv, None
+
+    class Pool:  # the host's copy of the pool's used end, by slot
+        def __getitem__(self, at):
+            return small[np.asarray(at) - shift * 64]
+
+    c.kv = Pool()
+    c.attn(d)
+    c.check_attn(_np(d["out"]), _np(d["lse"]))
+    acc = torch.zeros(n_pages * 64, device=cuda)
+    c.weights(d, acc)
+    at = np.concatenate([kv4.slots_of(c.bt, s, int(n)) for s, n in enumerate(c.lens)])
+    want, tol = c.want_weights(_np(d["lse"]).astype(np.float64))
+    err = np.abs(_np(acc)[at].astype(np.float64) - want[at])
+    assert np.all(err <= tol[at] + want[at] * 2.0 ** -24)
+    ind = torch.full((c.T, 2048), -1, dtype=torch.int32, device=cuda)
+    tlen = torch.full((c.T,), 130, dtype=torch.int32, device=cuda)
+    picks = [kv4.slots_of(c.bt, s, 130) for s in (0, 0, 1)]
+    for t in range(c.T):
+        ind[t, :130] = torch.from_numpy(picks[t].astype(np.int32)).to(cuda)
+    glmkv.kv4_attn_picks(d["q"], kv, n_pages, ind, tlen, 16, c.scale, d["out"], d["lse"], d["ws"], d["ws_bytes"], c.T)
+    c.check_attn(_np(d["out"]), _np(d["lse"]), rows_of=lambda t: picks[t])
+    kvd = torch.zeros(630, 576, dtype=torch.bfloat16, device=cuda)
+    glmkv.kv4_dequant(kv, d["bt"], c.max_pages, d["lens"], c.nseq, kvd)
+    assert np.array_equal(_np(kvd).astype(np.float64), np.concatenate(kv4.lift(c.kv[at]), 1))
+    # the last slots of the pool: an append into them, and moves between them
+    rng = np.random.default_rng(22)
+    w = W.weights(rng)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(cuda)
+    b = lambda a: t(a.view(np.int16)).view(torch.bfloat16)
+    x = b(W.bf16_bits(rng.standard_normal((8, 2624)).astype(np.float32)))
+    rows = {}
+    for name, pool, first in (("far", kv, n_pages * 64 - 8), ("near", torch.zeros(64, 416, dtype=torch.uint8, device=cuda), 0)):
+        qq, qsf = (torch.zeros(n, dtype=torch.uint8, device=cuda) for n in (8 * 2048, 16 * 8))
+        glmkv.mla_prep_shared(x, 2624, b(w.g_q), b(w.g_kv), b(W.rope_table(64)), torch.arange(8, dtype=torch.int32, device=cuda),
+                              torch.arange(first, first + 8, device=cuda), pool, qq, qsf, 8, 8, kv_dtype="fp4")
+        rows[name] = _np(pool[first:first + 8])
+    assert np.array_equal(rows["far"], rows["near"])
+    moves = torch.tensor([[[n_pages * 64 - 1, n_pages * 64 - 8], [n_pages * 64 - 2, n_pages * 64 - 7]]], dtype=torch.int32,
+                         device=cuda)
+    glmkv.evict_rows(moves, torch.tensor([2], dtype=torch.int32, device=cuda), 1, 2, n_pages, kv, None, None, None)
+    assert np.array_equal(_np(kv[-2:]), rows["near"][[1, 0]])
+    assert glmkv.fault_flags() == 0
+
+
 def test_same_bits_every_time(cuda):
     from kv4_case import Kv4Case
 
