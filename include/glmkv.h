@@ -32,6 +32,10 @@
  *   latent cache, 4 bits:     a token is 416 B: 512 e2m1 codes (value 2 j in the low nibble of byte j), 32
  *                             e4m3 scales (e4m3(amax / 6) of 16 values each), 64 bf16 roped k_pe; a lifted
  *                             value, code * scale, is exact in bf16 and f16. A page is 64 x 416 = 26624 B.
+ *                             The scales have none beside them: 16 values that are all below 6 * 2^-10 = 0.0059
+ *                             become zeros, below 6 * 2^-6 = 0.094 their scale has fewer than four bits, past
+ *                             2688 values saturate (an infinite one is 2688); fp8 rows, with f32 scales, have
+ *                             no such range. A NaN among the 16 makes all of them NaN.
  *   indexer cache:            a page of 64 tokens is 64 x 128 e4m3 keys, then their 64 f32 scales
  *                             (8448 B; 132 B a token).
  */
@@ -90,8 +94,8 @@ int glmkv_mla_prep_fp8(const void* x, int lda, const void* g_q, const void* g_kv
                        void* qq, void* qsf, int sf_rows, int T, glmkv_stream_t stream);
 
 /* The same append into the 4-bit latent cache. Same arguments and requirements as glmkv_mla_prep. The codes
- * are e2m1(kv_norm / scale), round to nearest even, saturating; zero where the scale is. No counterpart in
- * the reference. */
+ * are e2m1(kv_norm / scale), round to nearest even, saturating; zeros with the values' signs where the scale is
+ * zero. No counterpart in the reference. */
 int glmkv_mla_prep_fp4(const void* x, int lda, const void* g_q, const void* g_kv, const void* rope,
                        const int32_t* pos, const int64_t* slot, void* kv, void* idx, const void* ik_w, const void* ik_b,
                        void* qq, void* qsf, int sf_rows, int T, glmkv_stream_t stream);
@@ -126,7 +130,9 @@ int glmkv_kv4_workspace_bytes(int64_t* bytes);
  * sees nothing gets 0 and -inf. Rows at cu[nseq] and past it are not written. Tokens whose page is outside
  * 0 .. n_pages - 1, or past the table's max_pages, are skipped and flagged (fault bit 2). Any number of
  * heads up to 1024; 64 rows (query tokens x heads) of a sequence share one read of its cache. Runs on the
- * tensor cores (tcgen05, kind::f16, f32 sums). Two launches. Needs q, kv, out and ws 16-byte aligned,
+ * tensor cores (tcgen05, kind::f16, f32 sums), with q as f16 under a power of two a row (exact down to 2^-28 of the
+ * row's largest), its rope dims bf16, and the weights as f16 (off by 2^-12 of themselves, or by 2^-32 of the row's sum
+ * where they are small). |k_pe| up to 2^100 is in range. Two launches. Needs q, kv, out and ws 16-byte aligned,
  * ws_bytes >= glmkv_kv4_workspace_bytes. No counterpart in the reference. */
 int glmkv_kv4_attn(const void* q, const void* kv, int n_pages, const int32_t* block_table, int max_pages,
                    const int64_t* cu, const int32_t* seq_lens, int nseq, int heads, float scale, void* out,
@@ -140,10 +146,12 @@ int glmkv_kv4_attn_picks(const void* q, const void* kv, int n_pages, const int32
                          glmkv_stream_t stream);
 
 /* The weight each cached token got, added to its running sum: acc[slot] += the sum over the call's rows
- * that see it of exp(scale * q . k - lse[row]), for the q and lse of a glmkv_kv4_attn call (any lse [T,
- * heads] f32; rows with -inf add nothing). acc [n_pages * 64] f32 by slot. A token's sum is added once
- * and always in the same order; where sequences of one call share a page, once for each, in any order.
- * No counterpart in the reference. */
+ * that see it of exp(scale * q . k - lse[row]), for the q and lse of a glmkv_kv4_attn call over the same cache
+ * (any lse [T, heads] f32; rows with -inf add nothing). The lse of glmkv_kv4_attn_picks does not fit: a weight goes to
+ * every token that a row could see, picked or not, and together they may pass 1 by far. An f32 lse is off by
+ * 2^-24 of itself, and a weight by about 2^-22 of the row's largest score times itself: scores past some 10^5 give no
+ * usable weights. acc [n_pages * 64] f32 by slot. A token's sum is added once and always in the same order; where
+ * sequences of one call share a page, once for each, in any order. No counterpart in the reference. */
 int glmkv_kv4_weights(const void* q, const float* lse, const void* kv, int n_pages, const int32_t* block_table,
                       int max_pages, const int64_t* cu, const int32_t* seq_lens, int nseq, int heads, float scale,
                       float* acc, int T, glmkv_stream_t stream);
